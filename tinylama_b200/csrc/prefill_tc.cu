@@ -126,6 +126,15 @@ struct TileInfo {
     }
 };
 
+// Rows of a V tile behind the last position, which an earlier sequence left in the slot, to zero (by both P V
+// warps, before their products): their weight is zero, but zero times an infinity or a NaN is not.  Out
+// of line, to leave the issuing warps' loop as it is.
+__device__ __noinline__ void zero_leftovers(uint8_t *tile, int live, int rows, int lane) {
+    for (int e = live * 8 + lane; e < rows * 8; e += 32) *reinterpret_cast<uint4 *>(tile + e * 16) = make_uint4(0u, 0u, 0u, 0u);
+    fence_proxy_async_smem();
+    __syncwarp();
+}
+
 // Causal prefill, persistent: one CTA per SM walks work tiles (NQ*128 query rows of one
 // (sequence, q-head)) and keeps its TMEM, barriers and pipelines across them.
 //   warp 0: TMA (elected lane) -- Q of each tile into one of two Q buffers, K/V tiles into a ring
@@ -283,6 +292,7 @@ prefill_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constan
                     const int st = kvit % NS;
                     ok = wait_all(&bars->kv_full[st], (kvit / NS) & 1, p.err, abort_flag);
                     if (!ok) break;
+                    if (j == ti.nkv - 1 && j < ntq) zero_leftovers(sV + st * S_::KV_TILE, ti.off + p.ntok - j * BNK, BNK, lane);
                     if (j < ntq) {
                         // the tile's first P V overwrites O_q: the group has read the previous tile's out
                         if (j == 0 && nto > 0) ok = wait_all(&bars->o_free[q], (nto - 1) & 1, p.err, abort_flag);
