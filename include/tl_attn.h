@@ -221,8 +221,8 @@ TL_API int tl_check_device(tl_attn *h, void *stream);
 /* Device addresses of slot `slot` of layer `layer`: K and V, each [nHeadKv][maxLen][headDim] of the
  * cache's type (slots of a layer follow one another).  Valid until tl_attn_destroy. */
 TL_API int tl_kv_device(tl_attn *h, int layer, int slot, void **k, void **v);
-/* Grow the workspace to what tl_prefill_packed (nseq sequences, ntok rows) and tl_decode_shared
- * (nseq sequences) can need with any lengths and any prefix. */
+/* Grow the workspace to what tl_prefill_packed (up to nseq sequences and ntok rows) and
+ * tl_decode_shared (up to nseq sequences) can need with any lengths and any prefix. */
 TL_API int tl_packed_reserve(tl_attn *h, int nseq, int ntok);
 /* Norm, rotation and append of a packed batch in one pass.  q, k and v hold ntok rows of
  * nHead, nHeadKv and nHeadKv heads with ldq, ldk, ldv elements from row to row (column ranges of

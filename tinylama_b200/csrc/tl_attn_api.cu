@@ -1262,9 +1262,11 @@ int tl_packed_reserve(tl_attn *h, int nseq, int ntok) {
     if (ntok < 0) return fail(TL_ERR_INVALID, "negative number of rows");
     DeviceGuard g(h->device);
     return guarded([&] {
-        const size_t d = std::max(decode_shared_ws(h, nseq, TL_IO_F32, kMaxChunks).bytes,
-                                  decode_shared_ws(h, nseq, TL_IO_BF16, kMaxChunks).bytes);
-        return ensure_packed(h, std::max(d, packed_part_bytes(h)), h->stream);
+        // a smaller batch can need more: its prefix has fewer units and is cut into more parts
+        size_t d = packed_part_bytes(h);
+        for (int n = 1; n <= nseq; ++n)
+            for (const int io : {TL_IO_F32, TL_IO_BF16}) d = std::max(d, decode_shared_ws(h, n, io, kMaxChunks).bytes);
+        return ensure_packed(h, d, h->stream);
     });
 }
 
