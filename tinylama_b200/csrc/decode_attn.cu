@@ -357,21 +357,16 @@ size_t smem_t(int nseq) {
 }
 
 template <typename KV, int D, int G>
+SmemLimit g_limit;
+
+template <typename KV, int D, int G>
 cudaError_t launch_t(const DecodeArgs &a, int num_ctas, cudaStream_t s) {
     using C = DecCfg<KV, D, G>;
     const size_t smem = smem_t<KV, D, G>(a.nseq);
     auto kern = decode_kernel<KV, D, G>;
-    // set the shared-memory limit only when it grows, so that steady-state launches (and CUDA
-    // graph capture of them) make no attribute calls
-    static size_t smem_set[64] = {};  // per device: attributes are per context
-    int dev = 0;
-    cudaGetDevice(&dev);
-    size_t &cur = smem_set[dev & 63];
-    if (smem > cur) {
-        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (e != cudaSuccess) return e;
-        cur = smem;
-    }
+    // steady-state launches (and CUDA graph capture of them) make no attribute calls
+    const cudaError_t e = allow_smem(kern, smem, g_limit<KV, D, G>);
+    if (e != cudaSuccess) return e;
     return launch_pdl(kern, dim3(num_ctas), dim3(C::THREADS), smem, s, a);
 }
 
@@ -391,7 +386,7 @@ int occ_t(int nseq) {
     using C = DecCfg<KV, D, G>;
     int n = 0;
     const size_t smem = smem_t<KV, D, G>(nseq);
-    cudaFuncSetAttribute(decode_kernel<KV, D, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    allow_smem(decode_kernel<KV, D, G>, smem, g_limit<KV, D, G>);
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, decode_kernel<KV, D, G>, C::THREADS, smem) != cudaSuccess) n = 1;
     return n < 1 ? 1 : n;
 }

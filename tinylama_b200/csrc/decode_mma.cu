@@ -772,6 +772,9 @@ bool make_cache_map(CUtensorMap *m, const void *ptr, uint64_t rows, int D, bool 
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+template <typename KV, int D, int G, bool CLU>
+SmemLimit g_limit;
+
 template <typename KV, int D, int G>
 cudaError_t launch_t(const DecodeArgs &a, int num_ctas, cudaStream_t s) {
     using C = MmaCfg<KV, D, G>;
@@ -781,23 +784,10 @@ cudaError_t launch_t(const DecodeArgs &a, int num_ctas, cudaStream_t s) {
     if (!make_cache_map(&km, a.kv.k, rows, D, C::F32) || !make_cache_map(&vm, a.kv.v, rows, D, C::F32))
         return cudaErrorNotSupported;
     const size_t smem = C::smem_bytes(a.nseq);
-    int dev = 0;
-    cudaGetDevice(&dev);
-    // only when it grows (per device and kernel): steady-state launches make no attribute calls
-    auto ensure_smem = [&](auto kern, size_t *set) -> cudaError_t {
-        size_t &cur = set[dev & 63];
-        if (smem > cur) {
-            cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-            if (e != cudaSuccess) return e;
-            cur = smem;
-        }
-        return cudaSuccess;
-    };
     if (a.cluster > 0) {
         if (a.cluster > kMaxCluster || num_ctas % a.cluster != 0) return cudaErrorInvalidValue;
-        static size_t smem_set_clu[64] = {};
         auto kern = decode_mma_kernel<KV, D, G, true>;
-        cudaError_t e = ensure_smem(kern, smem_set_clu);
+        cudaError_t e = allow_smem(kern, smem, g_limit<KV, D, G, true>);
         if (e != cudaSuccess) return e;
         if (a.cluster > 8) {
             e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
@@ -805,9 +795,8 @@ cudaError_t launch_t(const DecodeArgs &a, int num_ctas, cudaStream_t s) {
         }
         return launch_pdl_cluster(kern, dim3(num_ctas), dim3(C::THREADS), smem, a.cluster, s, km, vm, a);
     }
-    static size_t smem_set[64] = {};
     auto kern = decode_mma_kernel<KV, D, G, false>;
-    cudaError_t e = ensure_smem(kern, smem_set);
+    cudaError_t e = allow_smem(kern, smem, g_limit<KV, D, G, false>);
     if (e != cudaSuccess) return e;
     return launch_pdl(kern, dim3(num_ctas), dim3(C::THREADS), smem, s, km, vm, a);
 }
@@ -818,7 +807,7 @@ int occ_t(int nseq) {
     int n = 0;
     const size_t smem = C::smem_bytes(nseq);
     auto kern = decode_mma_kernel<KV, D, G, false>;
-    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    allow_smem(kern, smem, g_limit<KV, D, G, false>);
     if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kern, C::THREADS, smem) != cudaSuccess)
         n = 1;
     return n < 1 ? 1 : n;
@@ -868,7 +857,7 @@ int cluster_capacity_t(int cluster) {
     using C = MmaCfg<KV, D, G>;
     const size_t smem = C::smem_bytes(512);  // at least what a cluster-mode launch uses (nseq <= 512)
     auto kern = decode_mma_kernel<KV, D, G, true>;
-    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return 0;
+    if (allow_smem(kern, smem, g_limit<KV, D, G, true>) != cudaSuccess) return 0;
     if (cluster > 8 && cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess) {
         cudaGetLastError();
         return 0;

@@ -415,9 +415,9 @@ cudaError_t launch_t(const OwnArgs &a, cudaStream_t s) {
     p.state = a.state;
     p.err = a.err;
     auto kern = decode_own_kernel<IO, KV, D>;
-    static int smem_set[64] = {};
+    static SmemLimit limit;
     const int smem = C::smem(a.nseq);
-    const cudaError_t e = allow_smem(kern, smem, smem_set);
+    const cudaError_t e = allow_smem(kern, smem, limit);
     if (e != cudaSuccess) return e;
     const int64_t jobs = (int64_t)a.nseq * p.nHeadKv * a.nchunks;
     if (jobs > INT32_MAX / 2) return cudaErrorNotSupported;

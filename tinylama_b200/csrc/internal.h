@@ -5,6 +5,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+#include <mutex>
 #include <string>
 #include <utility>
 #include <vector>
@@ -107,6 +109,27 @@ struct tl_attn {
 };
 
 namespace tl {
+
+// The dynamic shared memory that a kernel has been allowed, by device.  The attribute belongs to the
+// kernel, not to a call: every handle and host thread shares it, so it is only ever raised, under one
+// lock, and the size is published after it holds.
+struct SmemLimit {
+    std::atomic<int> bytes[64];
+};
+template <typename K>
+cudaError_t allow_smem(K kern, size_t smem, SmemLimit &limit) {
+    static std::mutex mu;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    std::atomic<int> &cur = limit.bytes[dev & 63];
+    if (cur.load(std::memory_order_acquire) >= (int)smem) return cudaSuccess;
+    std::lock_guard<std::mutex> lock(mu);
+    if (cur.load(std::memory_order_relaxed) >= (int)smem) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+    if (e == cudaSuccess) cur.store((int)smem, std::memory_order_release);
+    else cudaGetLastError();  // the caller reports it; it is not the next launch's
+    return e;
+}
 
 // Launch a kernel with programmatic stream serialisation: its CTAs may be scheduled while the
 // previous kernel on the stream still runs, and it waits (pdl_wait) before reading that

@@ -1003,10 +1003,9 @@ int tl_model_create(tl_model **out, const tl_model_config *cfg, int device) {
     // the largest gemv (kMaxS tokens of the ffn input) needs more than the default 48 KB
     const int big = std::max(c.nEmb, c.nFfn);
     const int smem = kMaxS * (xpad_len(big) + big / 16) * (int)sizeof(float);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(gemv_kernel<kMaxS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e == cudaSuccess)
-        e = cudaFuncSetAttribute(gemv_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                 (xpad_len(big) + big / 16) * (int)sizeof(float));
+    static SmemLimit limit_s, limit_1;
+    if (e == cudaSuccess) e = allow_smem(gemv_kernel<kMaxS>, smem, limit_s);
+    if (e == cudaSuccess) e = allow_smem(gemv_kernel<1>, (xpad_len(big) + big / 16) * sizeof(float), limit_1);
     // the pipelined Q2_K kernels take inputs up to 8192 wide
     const int smem1 = (xpad_len(8192) + 8192 / 16) * (int)sizeof(float), smem4 = kMaxS * smem1;
 #define TLM_ATTR(NS_, T_, SW_)                                                                             \

@@ -532,8 +532,8 @@ cudaError_t launch_t(const PackedArgs &a, cudaStream_t s) {
     }
     const int smem = S_::OFF_BARS + (int)sizeof(PkBars<D>) + 1024;
     auto kern = packed_tc_kernel<D>;
-    static int smem_set[64] = {};
-    const cudaError_t e = allow_smem(kern, smem, smem_set);
+    static SmemLimit limit;
+    const cudaError_t e = allow_smem(kern, smem, limit);
     if (e != cudaSuccess) return e;
     kern<<<a.ctas, kThreads, smem, s>>>(qm, km, vm, pkm, pvm, p);
     return cudaGetLastError();

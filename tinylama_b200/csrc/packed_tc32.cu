@@ -581,8 +581,8 @@ cudaError_t launch_t(const PackedArgs &a, cudaStream_t s) {
     }
     const int smem = C::OFF_BARS + (int)sizeof(P32Bars<D, KV32>) + 1024;
     auto kern = packed_tc32_kernel<D, KV32>;
-    static int smem_set[64] = {};
-    const cudaError_t e = allow_smem(kern, smem, smem_set);
+    static SmemLimit limit;
+    const cudaError_t e = allow_smem(kern, smem, limit);
     if (e != cudaSuccess) return e;
     kern<<<a.ctas, C::THREADS, smem, s>>>(km, vm, pkm, pvm, p);
     return cudaGetLastError();

@@ -522,14 +522,11 @@ cudaError_t launch_shape(const PrefillArgs &a, cudaStream_t s) {
     p.err = a.err;
     const int smem = S_::SMEM + (int)sizeof(Bars<NQ, S_::NS>) + 16 + NQ * 4 * kStgFloats * (int)sizeof(float) + 1024;
     auto kern = prefill_tc_kernel<NQ, BN_>;
-    static int smem_set[64] = {};
+    static SmemLimit limit;
+    const cudaError_t e = allow_smem(kern, smem, limit);
+    if (e != cudaSuccess) return e;
     int dev = 0;
     cudaGetDevice(&dev);
-    if (smem_set[dev & 63] < smem) {
-        cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (e != cudaSuccess) return e;
-        smem_set[dev & 63] = smem;
-    }
     // persistent: one CTA per SM (TMEM and shared memory allow one), at most one per tile
     static int sms[64] = {};
     if (sms[dev & 63] == 0) {

@@ -268,17 +268,5 @@ bool map_rows(CUtensorMap *m, const void *ptr, uint64_t rows, int D, bool f32, i
                CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-// Dynamic shared memory of a kernel, set only when it grows (per device)
-template <typename K>
-cudaError_t allow_smem(K kern, int smem, int *set) {
-    int dev = 0;
-    cudaGetDevice(&dev);
-    int &cur = set[dev & 63];
-    if (cur >= smem) return cudaSuccess;
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e == cudaSuccess) cur = smem;
-    return e;
-}
-
 }  // namespace
 }  // namespace tl
