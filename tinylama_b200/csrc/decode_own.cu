@@ -46,6 +46,7 @@ struct OwnCfg {
 
 struct OwnParams {
     const void *q;
+    const void *k, *v;    // from (layer, slot0) on
     const int *pos;
     int nseq, nHead, nHeadKv, G, max_len;
     int chunk, nchunks;   // positions per job, jobs per (sequence, kv-head)
@@ -64,6 +65,48 @@ __device__ __forceinline__ uint32_t third2(float x0, float x1, uint32_t hi, uint
     auto low = [](uint32_t u) { return __uint_as_float(u << 16); };
     auto high = [](uint32_t u) { return __uint_as_float(u & 0xffff0000u); };
     return pack2(x0 - low(hi) - low(lo), x1 - high(hi) - high(lo));
+}
+
+// The state of one head over a job's n positions (rows k, v) by fp32 products, for one whose sums have
+// come out not finite.  The matrix products take an infinity apart into parts (infinity - infinity) or
+// multiply it with a low part of zero, and both are NaN.  Here a key of minus infinity has no
+// weight, and an infinite value is what it is.  A warp takes a position at a time, D/32 columns a lane: about 25
+// instructions a position, some 20 times a head's share of the products above, and no further than
+// the first score that is not a number.
+template <typename IO, typename KV, int D>
+__device__ __noinline__ void own_again(const IO *q, const KV *k, const KV *v, int n, float *state, float2 *ml) {
+    constexpr int N = D / 32;
+    const int lane = threadIdx.x & 31;
+    const float scale = kLog2e / sqrtf((float)D);
+    q += lane * N;
+    k += lane * N;
+    v += lane * N;
+    float x[N], o[N], m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        x[i] = KvT<IO>::to_f(q[i]);
+        o[i] = 0.f;
+    }
+    for (int j = 0; j < n && l == l; ++j, k += D, v += D) {
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < N; ++i) s = fmaf(x[i], KvT<KV>::to_f(k[i]), s);
+#pragma unroll
+        for (int d = 16; d >= 1; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+        s *= scale;
+        if (s == -INFINITY) continue;
+        const float M = fmaxf(m, s), alpha = safe_exp2_diff(m, M), w = exp2f(s - M);
+        m = M;
+        l = fmaf(l, alpha, w);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            o[i] *= alpha;
+            if (w != 0.f) o[i] = fmaf(w, KvT<KV>::to_f(v[i]), o[i]);
+        }
+    }
+    if (lane == 0) *ml = make_float2(m, l);
+#pragma unroll
+    for (int i = 0; i < N; ++i) state[lane * N + i] = o[i];
 }
 
 template <typename IO, typename KV, int D>
@@ -362,11 +405,14 @@ decode_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
         if (!ok) break;
         // ---- the job's state, rows gid < G ----
         const int64_t rows = (int64_t)p.nseq * p.nHead, row = at.c * rows + head;
+        float z[4] = {l * 0.f, 0.f, 0.f, 0.f};  // NaN if a sum is not finite
         if (row_ok) {
             if (tq == 0) reinterpret_cast<float2 *>(p.state + p.nchunks * rows * D)[row] = make_float2(m, l);
             float *dst = p.state + row * D;
 #pragma unroll
             for (int nt = 0; nt < C::NT; ++nt) {
+                z[nt & 1] = fmaf(o[nt][0] + o[nt][2], 0.f, z[nt & 1]);
+                z[2 + (nt & 1)] = fmaf(o[nt][1] + o[nt][3], 0.f, z[2 + (nt & 1)]);
                 if constexpr (C::F32) {
                     const int c = 32 * (nt >> 2) + (nt & 3);  // column of n = 2tq is c + 8tq
                     dst[c + 8 * tq] = o[nt][0] + o[nt][2];
@@ -374,6 +420,18 @@ decode_own_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_constan
                 } else {
                     *reinterpret_cast<float2 *>(dst + 8 * nt + 2 * tq) = make_float2(o[nt][0] + o[nt][2], o[nt][1] + o[nt][3]);
                 }
+            }
+        }
+        const unsigned again = __ballot_sync(0xffffffffu, row_ok && (z[0] + z[1]) + (z[2] + z[3]) != 0.f);
+        if (again) {
+            __syncwarp();  // these rows are written once more
+            const int64_t first = (((int64_t)at.b * p.nHeadKv + at.g) * p.max_len + (int64_t)at.c * p.chunk) * D;
+            for (int r = 0; r < p.G; ++r) {
+                if (!(again >> (4 * r) & 15u)) continue;
+                const int64_t i = (int64_t)at.b * p.nHead + (int64_t)at.g * p.G + r;
+                own_again<IO, KV, D>(reinterpret_cast<const IO *>(p.q) + i * D, reinterpret_cast<const KV *>(p.k) + first,
+                                     reinterpret_cast<const KV *>(p.v) + first, at.n, p.state + (at.c * rows + i) * D,
+                                     reinterpret_cast<float2 *>(p.state + p.nchunks * rows * D) + at.c * rows + i);
             }
         }
         at = start(at.job + stride);
@@ -404,6 +462,8 @@ cudaError_t launch_t(const OwnArgs &a, cudaStream_t s) {
         return cudaErrorNotSupported;
     OwnParams p;
     p.q = a.q;
+    p.k = reinterpret_cast<const uint8_t *>(a.kv.k) + first;
+    p.v = reinterpret_cast<const uint8_t *>(a.kv.v) + first;
     p.pos = a.pos;
     p.nseq = a.nseq;
     p.nHead = a.nHead;
