@@ -208,8 +208,12 @@ TL_API int tl_check_device(tl_attn *h, void *stream);
  * prefixLen 0 means no prefix (prefix may then be NULL).
  *
  * ioType is the type of the activations (q, k, v, outputs).  TL_IO_BF16 needs a bf16 cache and
- * runs on the bf16 tensor cores with fp32 sums; TL_IO_F32 takes either cache and computes with
- * 32-bit products.  Other combinations are refused (TL_ERR_UNSUPPORTED).
+ * runs on the bf16 tensor cores with fp32 sums; the weights are rounded to bf16 (2^-8) before they
+ * meet V, except over the own positions of tl_decode_shared, where they keep 16 bits.  TL_IO_F32
+ * takes either cache and computes with 32-bit products: every operand in parts that hold its 24
+ * bits, except over the own positions of tl_decode_shared in an f32 cache, where q, K, the weights
+ * and V are held to 2^-22.  Sums, maxima and norms are in fp32.  Other combinations are refused
+ * (TL_ERR_UNSUPPORTED).
  *
  * The attention calls keep partial results and counters in a workspace of the handle, so two of
  * them on one handle must not overlap on the GPU, captured and replayed ones included: order them

@@ -76,3 +76,24 @@ def norm_rope_bound(y, size, dtype, D):
     and the rotation 2 more; then the output is rounded."""
     e32 = HALF[torch.float32]
     return size * ((D + 1) / 2 + 8) * e32 + HALF[dtype] * y.abs() + 1e-30
+
+
+# The root mean square error of 32-bit attention against the definition, relative to the output's, stays
+# below this.  The bound above is a worst case, some hundred times the error that roundings of random
+# sign add up to; bits that a kernel drops would pass it.  A weight's relative error: a score of a few
+# units (log2) is rounded some eight times on its way, each by 2^-24 / sqrt(3) of it in the mean, and
+# ln(2) of that reaches the weight: 1.5e-7.  Values that have lost all behind their 16th bit are off
+# by 2^-17 / sqrt(3) of the power of two above them, 0.75 of that relative to themselves: 3.3e-6, and
+# scores from such keys or queries by as much of a standard deviation above one.
+RMS32 = 2.0 ** -20
+
+
+def rms_error(got, want):
+    got, want = got.double(), want.double()
+    return float((got - want).square().mean().sqrt() / want.square().mean().sqrt())
+
+
+def two_parts(x):
+    """x rounded to the sum of two bf16 values."""
+    a = x.to(torch.bfloat16).to(x.dtype)
+    return a + (x - a).to(torch.bfloat16).to(x.dtype)

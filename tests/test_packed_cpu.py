@@ -62,3 +62,19 @@ def test_norm_definition():
     x = torch.tensor([[[3.0, 4.0]]], dtype=torch.float32)
     y, _ = ref.norm_rope(x, torch.tensor([2.0, 1.0]), 0.0, torch.zeros(1), torch.zeros(0), 0)
     assert torch.allclose(y, torch.tensor([[[6.0, 4.0]]], dtype=torch.float64) / np.sqrt(12.5))
+
+
+def test_the_rms_limit_sees_a_lost_part():
+    """Attention in 64 bits from operands that kept two bf16 parts of three is outside the limit, whichever
+    operand it is; the same in 32 bits throughout is inside."""
+    g = torch.Generator().manual_seed(3)
+    n, H, K, D = 96, 4, 2, 64
+    q = torch.randn(n, H, D, generator=g) * 1.5
+    k, v = (torch.randn(K, n, D, generator=g) for _ in range(2))
+    want, _, _ = ref.attention(q, k, v, 0)
+    for lost in ((ref.two_parts(q), k, v), (q, ref.two_parts(k), v), (q, k, ref.two_parts(v))):
+        assert ref.rms_error(ref.attention(*lost, 0)[0], want) > 2 * ref.RMS32
+    s = torch.einsum("nhd,hmd->nhm", q, k.repeat_interleave(H // K, 0)) / D ** 0.5
+    s = s.masked_fill((torch.arange(n)[None] > torch.arange(n)[:, None])[:, None], -float("inf"))
+    got = torch.einsum("nhm,hmd->nhd", torch.softmax(s, -1), v.repeat_interleave(H // K, 0))
+    assert ref.rms_error(got, want) < ref.RMS32 / 2

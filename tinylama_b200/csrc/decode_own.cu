@@ -13,7 +13,9 @@
 // than one job more than another.  One CTA per SM, kWarps warps of NS tiles of
 // 16 KB: 192 KB in flight.  The G heads of the group are rows of mma.sync fragments as in
 // decode_mma.cu: a bf16 cache takes q and the weights as bf16 high and low parts (rows 0-7 and 8-15
-// of one m16n8k16), an f32 cache takes q, K, the weights and V as tf32 high and low parts.  f32 activations over
+// of one m16n8k16), an f32 cache takes q, K, the weights and V as tf32 high and low parts, which hold a value to
+// 2^-22 (a third part would be two more products for each two; the error of 48 sequences of up to 300 behind 2000,
+// 32/8/128, is below that of a 32-bit softmax as it is).  f32 activations over
 // a bf16 cache take a third bf16 part in a product of its own: two hold 16 bits of q, which left an
 // error of 3.4e-6 where a 32-bit softmax has 5e-7 (48 sequences of up to 300, 32/8/128).  Such warp-level
 // products reach HBM speed with G <= 8 rows; the 128 rows of a tcgen05 tile would be mostly empty.
