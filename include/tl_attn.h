@@ -196,10 +196,11 @@ TL_API int tl_check_device(tl_attn *h, void *stream);
  * sequences in slots slot0..slot0+nseq-1 whose rows follow one another without padding: sequence
  * b owns rows cu_dev[b] .. cu_dev[b+1]-1 (cu_dev[0] = 0, never falling; a length may be 0), and its
  * row t stands at own position pos0_dev[b] + t, the cache position in its slot (pos0_dev NULL: all
- * start at 0).  Rows from cu_dev[nseq] up to ntok belong to no sequence: they are neither read nor
- * written.  cu_dev and pos0_dev are device arrays; a pair of them that does not fit ntok or maxLen
- * is reported by tl_check_device (position-out-of-range or bad-argument), and the rows it concerns
- * are not computed.
+ * start at 0).  Rows from cu_dev[nseq] up to ntok belong to no sequence: what they hold does not
+ * matter (they may be read: the buffers have ntok rows), and their outputs are left as they were.
+ * cu_dev and pos0_dev are device arrays; a pair of them that does not fit ntok or maxLen is
+ * reported by tl_check_device (position-out-of-range or bad-argument), and no row of its sequence
+ * is computed: outputs and cache are left as they were.
  *
  * A prefix is what all sequences of the batch begin with (a system prompt, a document): positions
  * 0..prefixLen-1 of slot prefixSlot of the handle `prefix`, which may be h itself or another handle

@@ -76,6 +76,19 @@ __device__ __forceinline__ void store_row(T *p, const float (&x)[N]) {
     }
 }
 
+// What is wrong with sequence b of the batch (then none of its rows is computed, as in the attention of
+// packed rows).
+__device__ __forceinline__ unsigned bad_seq(long long first, long long end, long long pos, int ntok, int max_len) {
+    if (end < first || first < 0 || end > ntok) return TL_DEVERR_BAD_ARG;
+    return end > first && (pos < 0 || pos + end - first > max_len) ? TL_DEVERR_POS_RANGE : 0u;
+}
+// Out of line, and before the warp holds anything: the first warps of a launch only.
+__device__ __noinline__ void report_bad(const int *cu, const int *pos0, int nseq, int ntok, int max_len, int64_t b, int64_t step,
+                                        unsigned *err) {
+    for (; b < nseq; b += step)
+        if (const unsigned bad = bad_seq(cu[b], cu[b + 1], pos0 ? pos0[b] : 0, ntok, max_len)) atomicOr(err, bad);
+}
+
 // UNI: a warp's heads of one turn are all q, all k or all v (nHead and nHeadKv are multiples of HPW),
 // so what they are is decided once for the warp.
 template <typename IO, typename KV, int D, bool UNI>
@@ -90,6 +103,8 @@ __global__ void __launch_bounds__(kWarps * 32, 8) norm_rope_kernel(const NormRop
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);  // known to be the same for its lanes
     const int64_t job = (int64_t)blockIdx.x * kWarps + warp;
     if (job >= (int64_t)a.ntok * parts) return;
+    if (job * 32 < a.nseq)
+        report_bad(a.cu, a.pos0, a.nseq, a.ntok, a.kv.maxLen, job * 32 + lane, (int64_t)a.ntok * parts * 32, a.err);
     const int tok = (int)(job / parts), part = (int)(job - (int64_t)tok * parts);
     const int t1 = part * HPW, step = parts * HPW, mine = lane / LPH;  // heads t1 + mine, + step, ...
     const IO *qr = reinterpret_cast<const IO *>(a.q) + tok * a.ldq + d;
@@ -114,13 +129,9 @@ __global__ void __launch_bounds__(kWarps * 32, 8) norm_rope_kernel(const NormRop
         lo += c * st;
         n = min(st, n - c * st);
     }
-    const int first = a.cu[lo], end = a.cu[a.nseq];
-    const long long at = (long long)(a.pos0 ? a.pos0[lo] : 0) + (tok - first);
-    const bool in = at >= 0 && at < a.kv.maxLen;
-    if (lane == 0 && end > a.ntok) atomicOr(a.err, TL_DEVERR_BAD_ARG);
-    if (tok < first || tok >= end) return;
-    if (lane == 0 && !in) atomicOr(a.err, TL_DEVERR_POS_RANGE);
-    const int pos = in ? (int)at : -1;
+    const int first = a.cu[lo], end = a.cu[lo + 1], pos0 = a.pos0 ? a.pos0[lo] : 0;
+    if (tok < first || tok >= end || bad_seq(first, end, pos0, a.ntok, a.kv.maxLen)) return;
+    const int pos = pos0 + (tok - first);
     // cos/sin of the pairs of this thread's columns, from the lanes that evaluated them
     float2 cs[N / 2];
     {
@@ -201,7 +212,7 @@ __global__ void __launch_bounds__(kWarps * 32, 8) norm_rope_kernel(const NormRop
 #pragma unroll
                     for (int k = 0; k < N; ++k) qo[hh * D + k] = KvT<IO>::from_f(y[k]);
                 }
-            } else if (pos >= 0 && kind < heads) {
+            } else if (kind < heads) {
                 const int h = hh - a.nHead - (is_k ? 0 : a.nHeadKv);
                 store_row<KV, N>(reinterpret_cast<KV *>(is_k ? a.kv.k : a.kv.v) + row0 + h * hs, y);
             }
