@@ -237,7 +237,8 @@ TL_API int tl_packed_reserve(tl_attn *h, int nseq, int ntok);
  * q_out [ntok][nHead*headDim]; k likewise with wk into the cache at own position pos0 + t, and v
  * into the cache as it is.  posBase is the length of the prefix, 0 without one.  theta (host
  * float[ropeDim/2], read during the call) replaces the handle's frequencies when not NULL.  q_out
- * may be q when ldq = nHead*headDim; other overlaps are not allowed. */
+ * may be q when ldq = nHead*headDim; any other overlap with rows of q, k or v is refused
+ * (TL_ERR_INVALID). */
 TL_API int tl_qk_norm_rope_append(tl_attn *h, int layer, int slot0, int nseq, int ntok, const int *cu_dev,
                                   const int *pos0_dev, int posBase, int ioType, const void *q, int ldq,
                                   const void *k, int ldk, const void *v, int ldv, const float *wq,

@@ -513,6 +513,14 @@ constexpr int kMaxAngle = 1 << 24;  // the rotation's positions are float32 valu
 
 bool aligned(const void *p, unsigned bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 
+// Does any of n rows (width bytes each, ld bytes apart) touch the `bytes` bytes at out?
+bool rows_touch(const void *rows, long long ld, long long width, int n, const void *out, long long bytes) {
+    const long long r0 = (long long)reinterpret_cast<uintptr_t>(rows), o0 = (long long)reinterpret_cast<uintptr_t>(out);
+    const long long before = o0 - r0 - width;             // a row that starts here or earlier ends before out
+    const long long r = before < 0 ? 0 : before / ld + 1;  // the first that does not
+    return r < n && r0 + r * ld < o0 + bytes;
+}
+
 int check_io(const tl_attn *h, int io) {
     if (io != TL_IO_F32 && io != TL_IO_BF16)
         return fail(TL_ERR_INVALID, "ioType %d is neither TL_IO_F32 nor TL_IO_BF16", io);
@@ -1290,6 +1298,11 @@ int tl_qk_norm_rope_append(tl_attn *h, int layer, int slot0, int nseq, int ntok,
     if (!aligned(q, es) || !aligned(k, es) || !aligned(v, es) || !aligned(q_out, es) || !aligned(wq, 4) || !aligned(wk, 4))
         return fail(TL_ERR_INVALID, "a pointer is not aligned to its element");
     if (q_out == q && ldq != Dq) return fail(TL_ERR_INVALID, "q_out may be q only when q's rows are contiguous");
+    // a warp reads its rows while others store theirs
+    const long long w = es, bytes = w * ntok * Dq;
+    if ((q_out != q && rows_touch(q, w * ldq, w * Dq, ntok, q_out, bytes)) || rows_touch(k, w * ldk, w * Dk, ntok, q_out, bytes) ||
+        rows_touch(v, w * ldv, w * Dk, ntok, q_out, bytes))
+        return fail(TL_ERR_INVALID, "q_out overlaps rows of q, k or v");
     if (ntok == 0) return TL_OK;
     DeviceGuard g(h->device);
     NormRopeArgs a{};
