@@ -220,8 +220,8 @@ TL_API int tl_check_device(tl_attn *h, void *stream);
  * them on one handle must not overlap on the GPU, captured and replayed ones included: order them
  * on one stream or by events, or use a handle per stream.  The workspace grows when a larger
  * batch comes; a call that would have to grow it while its stream is being captured is refused
- * (TL_ERR_INVALID): reserve it first.  What a captured graph uses stays valid until
- * tl_attn_destroy. */
+ * (TL_ERR_INVALID): reserve it first.  A workspace may grow while other streams are being
+ * captured.  What a captured graph uses stays valid until tl_attn_destroy. */
 
 /* Device addresses of slot `slot` of layer `layer`: K and V, each [nHeadKv][maxLen][headDim] of the
  * cache's type (slots of a layer follow one another).  Valid until tl_attn_destroy. */

@@ -148,7 +148,14 @@ int ensure_packed(tl_attn *h, size_t bytes, cudaStream_t s) {
     const size_t cap = std::max<size_t>(bytes + bytes / 2, 1 << 20);
     void *p = nullptr;
     h->packedOld.reserve(h->packedOld.size() + 1);
-    TL_CUDA(cudaMalloc(&p, cap));
+    // Another stream's capture, of this thread or (in the global mode) of any, must not be ended by the
+    // allocation, which is not part of it.
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    TL_CUDA(cudaThreadExchangeStreamCaptureMode(&mode));
+    const cudaError_t e = cudaMalloc(&p, cap);
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (e != cudaSuccess) cudaGetLastError();  // reported here, not by the next launch
+    TL_CUDA(e);
     if (h->dPacked) h->packedOld.push_back(h->dPacked);
     h->dPacked = p;
     h->packedCap = cap;
