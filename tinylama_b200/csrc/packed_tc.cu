@@ -29,7 +29,7 @@
 //
 // Masked keys.  A slot's rows behind the last position hold leftovers; the warps that issue P V set
 // those rows of V to zero in shared memory.  Values of the sequence itself that are not finite: see
-// redo_row (packed_tc.cuh).
+// clean_rows (packed_tc.cuh).
 //
 // Every mbarrier wait is bounded (common.cuh); TMEM is released on every path after all issued MMAs
 // have completed.
@@ -325,12 +325,19 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                     ok = wait_all(&bars->v_full[st], (kvit / NS) & 1, p.err, abort_flag);
                     if (!ok) break;
                     if (j < end) {
-                        zero_v(pc, j, sV + st * S_::TILE);
+                        uint8_t *vt = sV + st * S_::TILE;
+                        zero_v(pc, j, vt);
+                        const int seen = pc.pos + 1 - (j - p.in.prefix_tiles) * kKeyTile;  // own keys that every row sees
+                        if (p.in.cu != nullptr && j >= p.in.prefix_tiles && seen < kKeyTile) {
+                            unsigned bit;
+                            unsigned *word = bars->ring.bad_word(it, pc, j, bit);
+                            clean_rows<S_::HALVES, S_::BOX, 1>(vt, max(seen, 0), min(seen - 1 + pc.ntok, kKeyTile), word, bit);
+                        }
                         if (j == pc.j0 && nto > 0) ok = wait_all(&bars->o_free[q], (nto - 1) & 1, p.err, abort_flag);
                         if (ok) ok = wait_all(&bars->p_ready[q], npv & 1, p.err, abort_flag);
                         if (!ok) break;
                         tc_fence_after();
-                        const uint32_t va = smem_u32(sV + st * S_::TILE);
+                        const uint32_t va = smem_u32(vt);
 #pragma unroll
                         for (int kb = 0; kb < kKeyTile / 64; ++kb)
                             mma_pv_k64(tmem + S_::col_o(q), tmem + S_::col_p(q) + kb * 32,
@@ -483,7 +490,7 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
 #pragma unroll
                 for (int d = 0; d < D; ++d) o[d] = 0.f;
             }
-            redo_row<D, D, false, __nv_bfloat16, __nv_bfloat16>(p, pc, q * BM + r, 0, C, m_run, l, o);
+            put_back<D, D, false, __nv_bfloat16>(p, pc, bars->ring.bad[it % kRing], bars->ring.bad_step(pc), q * BM + r, 0, o);
             ok = finish_rows<D, D, __nv_bfloat16, 2 * BM>(p, cut, pc, q, q * BM + r, 0, o, m_run, l, group_sync,
                                                           &bars->last_flag[q],
                                                           base + S_::OFF_STG + (warp - 4) * 32 * kStgRow);

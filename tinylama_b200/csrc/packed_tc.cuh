@@ -107,6 +107,7 @@ template <int CONSUMERS>
 struct PieceRing {
     uint64_t full[kRing], empty[kRing];
     Piece slot[kRing];
+    unsigned bad[kRing][2];  // see clean_rows
     __device__ __forceinline__ void init() {
         for (int i = 0; i < kRing; ++i) {
             mbar_init(&full[i], 1);
@@ -119,6 +120,7 @@ struct PieceRing {
         if (!__all_sync(0xffffffffu, mbar_wait(&empty[i], ((it / kRing) & 1) ^ 1, err, ab))) return false;
         if (leader) {
             slot[i] = pc;
+            bad[i][0] = bad[i][1] = 0u;
             mbar_arrive(&full[i]);
         }
         __syncwarp();
@@ -132,6 +134,13 @@ struct PieceRing {
             return nullptr;
         }
         return slot[i].w < 0 ? nullptr : &slot[i];
+    }
+    // a bit for every 1/64 of a piece's tiles (at least one): the word and the bit of tile j
+    __device__ __forceinline__ static int bad_step(const Piece &pc) { return (pc.j1 - pc.j0 + 63) >> 6; }
+    __device__ __forceinline__ unsigned *bad_word(int it, const Piece &pc, int j, unsigned &bit) {
+        const int b = (j - pc.j0) / bad_step(pc);
+        bit = 1u << (b & 31);
+        return &bad[it % kRing][b >> 5];
     }
     __device__ __forceinline__ void put(int it, int lane) {
         __syncwarp();
@@ -198,78 +207,127 @@ __device__ __forceinline__ void load_floats(const T *p, float (&x)[N]) {
     }
 }
 
-// A value of V that is infinite or not a number reaches, in the matrix products, every row of its tile:
-// the weight of a row that does not see the key is zero, but zero times infinity is not.  (And the
-// parts of an infinity, in K too, cancel to NaN in the f32 kernel.)  Rows of V behind the last position are
-// zeroed before they are used; for the others nothing is checked on the way.  Instead a row whose sum
-// has come out not finite is summed again here, in fp32 on the CUDA cores, over the keys that it sees;
-// for f32 activations (PARTS) its maximum and its sum of weights too, where those are not a number
-// although q is finite.  That is slow, and happens only where such values are about.
-template <int D, int W, bool PARTS, typename IO, typename KV>
-__device__ __forceinline__ void redo_row(const PkParams<D> &p, const Piece &pc, int row, int col0, float scale, float &m,
-                                         float &l, float (&o)[W]) {
-    float z0 = 0.f, z1 = 0.f;  // NaN if a value is not finite
+// Values that are not finite.  In the matrix products a value of V that is infinite or not a number reaches every
+// row of its tile: the weight of a row that does not see the key is zero, but zero times infinity is
+// not.  So such values are set to zero in shared memory before the product, and their tile is marked; when a piece
+// ends, each row adds those that it sees to its sum as they are (put_back).  Looked over are the keys that
+// not every row of the unit sees, at most as many as the unit has tokens: the others are right as they are.  Of
+// f32 activations over a bf16 cache all keys are: their weights come in parts of either sign, which makes NaN of
+// an infinity also for the rows that see it.
+// So the cost is bounded whatever the values.  8 documents of up to 4096 (32/8/64 bf16): a NaN in each one's first
+// position takes no time (summing the rows again on the CUDA cores, each over all its keys, took 80 ms), NaN
+// everywhere 1.2 ms instead of 0.47; the most is a bf16 cache under f32 activations, 4 prompts of up to 1024 (32/4/64):
+// 14 times the 80 us with one such value in every tile of V, 29 times with a minus infinity in every key.
+
+// four words of two bf16 values each: not a number (in one of two halves) if one of them is not finite
+__device__ __forceinline__ uint32_t not_finite(uint4 u, uint32_t z) {
+    const __nv_bfloat162 zero = __floats2bfloat162_rn(0.f, 0.f);
+    __nv_bfloat162 a = *reinterpret_cast<__nv_bfloat162 *>(&z);
+    a = __hfma2(*reinterpret_cast<__nv_bfloat162 *>(&u.x), zero, a);
+    a = __hfma2(*reinterpret_cast<__nv_bfloat162 *>(&u.y), zero, a);
+    a = __hfma2(*reinterpret_cast<__nv_bfloat162 *>(&u.z), zero, a);
+    a = __hfma2(*reinterpret_cast<__nv_bfloat162 *>(&u.w), zero, a);
+    return *reinterpret_cast<uint32_t *>(&a);
+}
+constexpr uint32_t kNotZero = 0x7fff7fffu;  // bits of such a word that a zero of either sign does not have
+
+// bits of the values of a pair that are finite
+__device__ __forceinline__ uint32_t finite_halves(uint32_t u) {
+    return ((u & 0x7f80u) != 0x7f80u ? 0xffffu : 0u) | ((u & 0x7f800000u) != 0x7f800000u ? 0xffff0000u : 0u);
+}
+
+// Rows r0 .. r1-1 of a bf16 V tile, by a warp (two may do it at a time): values that are not finite to zero, and
+// the tile's mark.  UNROLL > 1 takes fewer turns, but more of the instruction cache: bf16, 8 documents of up
+// to 4096 (32/8/64) take 461 us with 1, 501 with 2, 512 with 4.
+template <int HALVES, int BOX, int UNROLL>
+__device__ __forceinline__ void clean_rows(uint8_t *tile, int r0, int r1, unsigned *word, unsigned bit) {
+    const int lane = threadIdx.x & 31;
+    uint32_t z[2] = {0u, 0u};
 #pragma unroll
-    for (int d = 0; d < W; d += 2) {
-        z0 = fmaf(o[d], 0.f, z0);
-        z1 = fmaf(o[d + 1], 0.f, z1);
-    }
-    const int tok = row >> p.lg_g;
-    const bool lost = l != l;
-    if ((z0 + z1 == 0.f && !lost) || tok >= pc.ntok || (lost && !PARTS)) return;
-    const int64_t qrow = (int64_t)(pc.tok0 + tok) * p.nHead + (pc.g << p.lg_g) + (row & ((1 << p.lg_g) - 1));
-    const IO *q = reinterpret_cast<const IO *>(p.q) + qrow * D;
-    constexpr int NQ = 16 / (int)sizeof(IO), NK = 16 / (int)sizeof(KV);
-    // f(s, v row) for every key that the row sees
-    auto keys = [&](auto f) {
-        for (int j = pc.j0; j < pc.j1; ++j) {
-            const bool pre = j < p.in.prefix_tiles;
-            const int k0 = (pre ? j : j - p.in.prefix_tiles) << p.in.lg_kt;
-            const int n = min(1 << p.in.lg_kt, (pre ? p.prefix_len : pc.pos + tok + 1) - k0);
-            const int64_t first = (pre ? (int64_t)pc.g * p.prefix_max_len
-                                       : ((int64_t)pc.b * p.in.heads_kv + pc.g) * p.in.max_len) + k0;
-            const KV *kc = reinterpret_cast<const KV *>(pre ? p.pk : p.k) + first * D;
-            const KV *vc = reinterpret_cast<const KV *>(pre ? p.pv : p.v) + first * D;
-            for (int i = 0; i < n; ++i, kc += D, vc += D) {
-                float s = 0.f;
+    for (int hh = 0; hh < HALVES; ++hh)
+#pragma unroll UNROLL
+        for (int e = r0 * 8 + lane; e < r1 * 8; e += 32)
+            z[hh] = not_finite(*reinterpret_cast<const uint4 *>(tile + hh * BOX + e * 16), z[hh]);
+    // (marked already: by the other warp, whose zeros this one may have found; they go to the product by this fence)
+    if (__any_sync(0xffffffffu, ((z[0] | z[1]) & kNotZero) != 0u || (*reinterpret_cast<volatile unsigned *>(word) & bit))) {
+        if (lane == 0) atomicOr(word, bit);
+        __threadfence_block();  // the mark before the zeros
+        __syncwarp();
 #pragma unroll 1
-                for (int d = 0; d < D; d += 8) {
-                    float x[8], y[8];
+        for (int hh = 0; hh < HALVES; ++hh)
+#pragma unroll 1
+            for (int e = r0 * 32 + lane; e < r1 * 32; e += 32) {
+                uint32_t *w = reinterpret_cast<uint32_t *>(tile + hh * BOX + e * 4);
+                const uint32_t keep = finite_halves(*w);
+                if (keep != ~0u) *w &= keep;
+            }
+        fence_proxy_async_smem();
+        __syncwarp();
+    }
+}
+
+// The same for a V tile in three parts, without the mark: of a value that is not finite, the third part is not.
+template <int HALVES, int BOX, int PART>
+__device__ __noinline__ void clean_parts(uint8_t *tile, int r0, int r1) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll 1
+    for (int hh = 0; hh < HALVES; ++hh)
+#pragma unroll 1
+        for (int e = r0 * 32 + lane; e < r1 * 32; e += 32) {
+            uint32_t *w = reinterpret_cast<uint32_t *>(tile + hh * BOX + e * 4);
+            const uint32_t keep = finite_halves(w[2 * PART / 4]);
+            if (keep == ~0u) continue;
+            for (int k = 0; k < 3; ++k) w[k * PART / 4] &= keep;
+        }
+    fence_proxy_async_smem();
+    __syncwarp();
+}
+
+// The cleaned values that row `row` of the unit sees, columns col0 .. col0+W-1, into its sum.  (Their weight
+// is taken as positive: one that underflows to zero would make NaN of an infinity.)
+template <int D, int W, bool ALL, typename KV>
+__device__ __forceinline__ void put_back(const PkParams<D> &p, const Piece &pc, const volatile unsigned *bad, int step, int row,
+                                         int col0, float (&o)[W]) {
+    constexpr int NK = 16 / (int)sizeof(KV);
+    const unsigned w0 = bad[0], w1 = bad[1];
+    if ((w0 | w1) == 0u) return;
+    const int tok = row >> p.lg_g;
+    if (tok >= pc.ntok) return;
+    for (int j = pc.j0; j < pc.j1; ++j) {
+        const int b = (j - pc.j0) / step;
+        if (!((b < 32 ? w0 : w1) >> (b & 31) & 1u)) continue;
+        const bool pre = j < p.in.prefix_tiles;
+        const int k0 = (pre ? j : j - p.in.prefix_tiles) << p.in.lg_kt;
+        const int n = min(1 << p.in.lg_kt, (pre ? p.prefix_len : pc.pos + tok + 1) - k0);
+        const int64_t first = (pre ? (int64_t)pc.g * p.prefix_max_len : ((int64_t)pc.b * p.in.heads_kv + pc.g) * p.in.max_len) + k0;
+        const KV *v = reinterpret_cast<const KV *>(pre ? p.pv : p.v) + first * D + col0;
+        for (int i = ALL ? 0 : pre ? n : max(pc.pos + 1 - k0, 0); i < n; ++i) {
 #pragma unroll
-                    for (int c = 0; c < 8; c += NQ) load_floats<IO, NQ>(q + d + c, *reinterpret_cast<float(*)[NQ]>(x + c));
+            for (int d = 0; d < W; d += NK) {
+                float x[NK];
+                load_floats<KV, NK>(v + (int64_t)i * D + d, x);
 #pragma unroll
-                    for (int c = 0; c < 8; c += NK) load_floats<KV, NK>(kc + d + c, *reinterpret_cast<float(*)[NK]>(y + c));
-#pragma unroll
-                    for (int c = 0; c < 8; ++c) s = fmaf(x[c], y[c], s);
-                }
-                f(s * scale, vc + col0);
+                for (int c = 0; c < NK; ++c) o[d + c] += fabsf(x[c]) < INFINITY ? 0.f : x[c];
             }
         }
-    };
-    if (PARTS && lost) {
-        float zq = 0.f;
-#pragma unroll 1
-        for (int d = 0; d < D; ++d) zq = fmaf(KvT<IO>::to_f(q[d]), 0.f, zq);
-        if (zq != 0.f) return;  // q itself is not finite
-        m = -INFINITY;
-        keys([&](float s, const KV *) { m = fmaxf(m, s); });
-        l = 0.f;
-        // a score of +infinity, or none, makes the sum NaN, as it is
-        keys([&](float s, const KV *) { l += s == -INFINITY ? 0.f : exp2f(s - m); });
     }
+}
+
+// Is the score of q and a key that has come out not a number minus infinity?  Only elements of the key that
+// are not finite count.
+template <int D, typename KV>
+__device__ __noinline__ bool weightless(const float *q, const KV *k) {
+    constexpr int NK = 16 / (int)sizeof(KV);
+    float s = 0.f;
+#pragma unroll 1
+    for (int d = 0; d < D; d += NK) {
+        float x[NK];
+        load_floats<KV, NK>(k + d, x);
 #pragma unroll
-    for (int d = 0; d < W; ++d) o[d] = 0.f;
-    keys([&](float s, const KV *v) {
-        const float w = exp2f(s - m);
-        if (!(w > 0.f)) return;
-#pragma unroll
-        for (int d = 0; d < W; d += NK) {
-            float x[NK];
-            load_floats<KV, NK>(v + d, x);
-#pragma unroll
-            for (int c = 0; c < NK; ++c) o[d + c] = fmaf(w, x[c], o[d + c]);
-        }
-    });
+        for (int c = 0; c < NK; ++c)
+            if (!(fabsf(x[c]) < INFINITY)) s = fmaf(q[d + c], x[c], s);
+    }
+    return s == -INFINITY;
 }
 
 // Called by 128 threads that hold columns col0 .. col0+W-1 of rows 128*n .. 128*n+127 of a unit of ROWS

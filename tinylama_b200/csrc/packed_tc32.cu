@@ -18,7 +18,10 @@
 // one tile) D: 480 for both head sizes.
 //   warp 0     derives the pieces of work, and brings K and V tiles of a bf16 cache (TMA)
 //   warp 1     issues S(j+1) = Q K^T, then T(j) = P V
-//   warp 3     bf16 cache: zeroes the rows of a V tile that hold leftovers
+//   warp 3     bf16 cache: zeroes the rows of a V tile that hold leftovers, and values that are not finite;
+//              f32 cache: looks over, in the cache, the new V rows of which not every row of a unit sees all, and
+//              tells warp 1, which cleans the tile (once for each such tile: with a turn of this warp on every tile
+//              the softmax lost issue slots to it, 111 us against 104, 4 prompts of up to 1024, 32/4/64)
 //   warps 4-7  f32 cache: read K and V, split them and write the parts in the swizzled layout (8 warps for
 //              it took registers from the softmax: 557 us against 451, 8 x up to 2048, 32/8/64)
 //   the last 8 softmax, two threads a row (half the keys of a tile, and half the columns of T, each; they
@@ -32,8 +35,10 @@
 // 260 for 4 of up to 2048 (32/8/128); the tensor pipe is 39% busy in the first (55% on the busiest SM), and waits
 // for the parts that the softmax threads write.
 //
-// Masked keys and leftovers: V rows that no row of the unit sees are zero in shared memory; values of the
-// sequence itself that are not finite: see redo_row (packed_tc.cuh).
+// Masked keys and leftovers: V rows that no row of the unit sees are zero in shared memory.  Values of the
+// sequence itself that are not finite: an f32 cache's infinities go through the products as what they are
+// (split3_cache), a bf16 cache's meet parts of either sign and are looked after (clean_rows in packed_tc.cuh for V,
+// keep_weights for K).
 #include <type_traits>
 
 #include "packed_tc.cuh"
@@ -53,15 +58,16 @@ struct P32 {
     static constexpr int CONV = KV32 ? 128 : 0;      // threads that split K and V
     static constexpr int THREADS = 384 + CONV;
     static constexpr int SOFT0 = THREADS / 32 - 8;   // first softmax warp
-    static constexpr int CONSUMERS = KV32 ? 1 + CONV / 32 + 8 : 1 + 1 + 8;  // warps that read the ring of pieces
+    static constexpr int CONSUMERS = 1 + 1 + CONV / 32 + 8;  // warps that read the ring of pieces
     static constexpr int OFF_V = NS * TILE;
     static constexpr int OFF_STG = 2 * NS * TILE;
     static constexpr int OFF_BARS = OFF_STG + 8 * 32 * kStgRow;
     static constexpr int COL_Q = 0, COL_S = 3 * D / 2, COL_P = COL_S + KT, COL_T = COL_P + 3 * KT / 2;
     static_assert(COL_T + D <= 512, "TMEM columns");
     // registers of the warpgroups: dec only goes down and inc only up, and together they stay within the
-    // launch's
-    static constexpr int REG_LAUNCH = 65536 / THREADS / 8 * 8, REG_CTRL = KV32 ? 64 : 104, REG_CONV = 104,
+    // launch's.  112 for the warps that split an f32 cache at headDim 128 (4 prompts of up to 2048, 32/8: 452 us
+    // against 482 with 104), 104 at 64 (8 of up to 2048, 32/8: 437 against 441 with 112).
+    static constexpr int REG_LAUNCH = 65536 / THREADS / 8 * 8, REG_CTRL = KV32 ? 64 : 104, REG_CONV = D == 64 ? 104 : 112,
                          REG_SOFT = KV32 ? 168 : 200;
     static_assert(REG_CTRL <= REG_LAUNCH && REG_CONV <= REG_LAUNCH && REG_SOFT >= REG_LAUNCH, "direction of the change");
     static_assert(REG_CTRL + CONV / 128 * REG_CONV + 2 * REG_SOFT <= THREADS / 128 * REG_LAUNCH,
@@ -72,12 +78,13 @@ template <int D, bool KV32>
 struct P32Bars {
     static constexpr int NS = P32<D, KV32>::NS;
     uint64_t k_full[NS], k_empty[NS], v_raw[NS], v_full[NS], v_empty[NS];
-    uint64_t q_ready, s_full, s_free, p_ready, o_bar, x_bar, g_bar[2], mma_final;
+    uint64_t v_clean, v_taken, q_ready, s_full, s_free, p_ready, o_bar, x_bar, g_bar[2], mma_final;
     PieceRing<P32<D, KV32>::CONSUMERS> ring;
     SchedStart start;
     uint32_t tmem_base;
     int abort;
     int last_flag[2];
+    volatile int verdict;  // rows of a V tile that are to be cleaned, or 0
     float xch[2][2][BM];  // a row's maximum (or sum) over each half of the keys, two turns of it
 };
 
@@ -109,6 +116,46 @@ __device__ __forceinline__ void split3(float x0, float x1, uint32_t &a, uint32_t
     b = pack_bf16(r.x, r.y);
     const float2 q = fsub2(r, make_float2(__uint_as_float(b << 16), __uint_as_float(b & 0xffff0000u)));
     c = pack_bf16(q.x, q.y);
+}
+
+// The same for values of the cache, of which an infinity has to stay one: the first two parts are clamped to the
+// largest bf16 value, so that only the third is infinite.  It meets only the first part of q or of the weights,
+// whose sign is theirs: a score or a sum comes out as the infinity that it is.  (A finite value that rounds to
+// infinity in bf16 is the exact sum of its clamped parts.)
+__device__ __forceinline__ uint32_t pack_clamped(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.satfinite.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ void split3_cache(float x0, float x1, uint32_t &a, uint32_t &b, uint32_t &c) {
+    a = pack_clamped(x0, x1);
+    const float2 r = fsub2(make_float2(x0, x1), make_float2(__uint_as_float(a << 16), __uint_as_float(a & 0xffff0000u)));
+    b = pack_clamped(r.x, r.y);
+    const float2 q = fsub2(r, make_float2(__uint_as_float(b << 16), __uint_as_float(b & 0xffff0000u)));
+    c = pack_bf16(q.x, q.y);
+}
+
+// A row's weights w of KH keys, of which some are not a number (`lost`; all lanes of the warp take part).  Such a
+// key has no weight if its score is minus infinity; then w and their sum are put right, and the result is true.
+// Otherwise the row has no softmax: the sum stays what it is, and the row is not looked at again.
+template <int D, int KH, typename KV>
+__device__ __noinline__ bool keep_weights(uint32_t *w, bool lost, const float *q, const KV *k, float &sum) {
+    bool none = false;
+    float s = 0.f;
+#pragma unroll 1
+    for (int c = 0; c < KH; ++c) {
+        const float x = __uint_as_float(w[c]);
+        const bool mine = lost && x != x;
+        if (__any_sync(0xffffffffu, mine && !none)) {
+            const bool out = weightless<D, KV>(q, k + (int64_t)c * D);
+            none |= mine && !out;
+        }
+        if (mine) w[c] = 0u;
+        else s += x;
+    }
+    if (!lost || none) return false;
+    sum = s;
+    return true;
 }
 
 // The terms of a product, small ones first: the parts of A and of B, four bits each from the low end.
@@ -164,6 +211,8 @@ packed_tc32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
             mbar_init(&bars->v_full[i], KV32 ? C::CONV / 32 : 1);
             mbar_init(&bars->v_empty[i], 1);
         }
+        mbar_init(&bars->v_clean, 1);
+        mbar_init(&bars->v_taken, 1);
         mbar_init(&bars->q_ready, 8);
         mbar_init(&bars->s_full, 1);
         mbar_init(&bars->s_free, 8);
@@ -208,6 +257,11 @@ packed_tc32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
         t.n = min(KT, (t.pre ? p.prefix_len : pc.pos + pc.ntok) - t.k0);
         t.all = t.pre ? KT : pc.pos + 1 - t.k0;
         return t;
+    };
+
+    // the first tile of which not every row of the unit sees every key
+    auto first_diagonal = [&](const Piece &pc) {
+        return p.in.cu != nullptr && pc.ntok > 1 ? p.in.prefix_tiles + ((pc.pos + 1) >> p.in.lg_kt) : pc.j1;
     };
 
     if (warp < 4) {
@@ -259,6 +313,7 @@ packed_tc32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
             const uint32_t idesc_s = idesc_bf16(KT, false), idesc_o = idesc_bf16(D, true);
             using T_ = Terms<C::NP>;
             int it = 0, ks = 0, ps = 0;  // pieces, S tiles issued, P V tiles issued
+            int diag = 0;                // tiles that warp 3 has had a say on
             bool ok = true;
             // S of the next tile
             auto issue_s = [&]() {
@@ -285,6 +340,7 @@ packed_tc32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                 const Piece *slot = bars->ring.get(it, p.err, abort_flag, &ok);
                 if (!slot) break;
                 const int n = slot->j1 - slot->j0;
+                const int clean = KV32 ? first_diagonal(*slot) - slot->j0 : n;  // the first tile that warp 3 has a say on
                 bars->ring.put(it, lane);
                 ok = wait_all(&bars->q_ready, it & 1, p.err, abort_flag);
                 if (!ok) break;
@@ -294,6 +350,13 @@ packed_tc32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                     if (!ok) break;
                     const int st = ps % NS;
                     ok = wait_all(&bars->v_full[st], (ps / NS) & 1, p.err, abort_flag);
+                    if (ok && j >= clean) {
+                        ok = wait_all(&bars->v_clean, diag++ & 1, p.err, abort_flag);
+                        const int verdict = bars->verdict;
+                        __syncwarp();
+                        if (ok && leader) mbar_arrive(&bars->v_taken);
+                        if (ok && verdict != 0) clean_parts<C::HALVES, C::BOX, C::PART>(sV + st * C::TILE, verdict >> 16, verdict & 0xffff);
+                    }
                     if (ok) ok = wait_all(&bars->p_ready, ps & 1, p.err, abort_flag);
                     if (!ok) break;
                     tc_fence_after();
@@ -313,29 +376,61 @@ packed_tc32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
             }
             tc_commit(&bars->mma_final, leader);
             wait_all(&bars->mma_final, 0, p.err, nullptr);
-        } else if (warp == 3 && !KV32) {
-            // ---------------- leftovers in V tiles ----------------
-            int kvit = 0, it = 0;
+        } else if (warp == 3) {
+            // ---------------- leftovers and values that are not finite in V tiles ----------------
+            int kvit = 0, it = 0, diag = 0;
             bool ok = true;
             for (; ok; ++it) {
                 const Piece *slot = bars->ring.get(it, p.err, abort_flag, &ok);
                 if (!slot) break;
                 const Piece pc = *slot;
                 bars->ring.put(it, lane);
-                for (int j = pc.j0; j < pc.j1; ++j, ++kvit) {
-                    const TileAt t = tile_at(pc, j);
-                    const int st = kvit % NS;
-                    if (!wait_all(&bars->v_raw[st], (kvit / NS) & 1, p.err, abort_flag)) { ok = false; break; }
-                    if (t.n < KT) {
-                        uint8_t *vt = sV + st * C::TILE;
-#pragma unroll
-                        for (int hh = 0; hh < C::HALVES; ++hh)
-                            for (int e = t.n * 8 + lane; e < KT * 8; e += 32)
-                                *reinterpret_cast<uint4 *>(vt + hh * C::BOX + e * 16) = make_uint4(0u, 0u, 0u, 0u);
-                        fence_proxy_async_smem();
+                if constexpr (KV32) {
+                    // Only tiles of which not every row sees every key, and from the cache itself, ahead of their
+                    // conversion: warp 1 takes the verdict when it comes to such a tile, and cleans it if need be.
+                    for (int j = max(pc.j0, first_diagonal(pc)); j < pc.j1 && ok; ++j, ++diag) {
+                        const TileAt t = tile_at(pc, j);
+                        const int from = max(t.all, 0);
+                        const uint4 *src = reinterpret_cast<const uint4 *>(reinterpret_cast<const float *>(p.v) + (t.row + from) * D);
+                        float z = 0.f;
+#pragma unroll 2
+                        for (int e = lane; e < (t.n - from) * (D / 4); e += 32) {
+                            const uint4 u = __ldg(src + e);
+                            z = fmaf(__uint_as_float(u.x), 0.f, fmaf(__uint_as_float(u.y), 0.f, z));
+                            z = fmaf(__uint_as_float(u.z), 0.f, fmaf(__uint_as_float(u.w), 0.f, z));
+                        }
+                        const bool bad = __any_sync(0xffffffffu, z != 0.f);
+                        ok = wait_all(&bars->v_taken, (diag & 1) ^ 1, p.err, abort_flag);
+                        if (ok && lane == 0) {
+                            bars->verdict = bad ? from << 16 | t.n : 0;
+                            if (bad) {
+                                unsigned bit;
+                                unsigned *word = bars->ring.bad_word(it, pc, j, bit);
+                                atomicOr(word, bit);
+                            }
+                            mbar_arrive(&bars->v_clean);
+                        }
                     }
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&bars->v_full[st]);
+                } else {
+                    for (int j = pc.j0; j < pc.j1 && ok; ++j, ++kvit) {
+                        const TileAt t = tile_at(pc, j);
+                        const int st = kvit % NS;
+                        uint8_t *vt = sV + st * C::TILE;
+                        ok = wait_all(&bars->v_raw[st], (kvit / NS) & 1, p.err, abort_flag);
+                        if (!ok) break;
+                        if (t.n < KT) {
+#pragma unroll
+                            for (int hh = 0; hh < C::HALVES; ++hh)
+                                for (int e = t.n * 8 + lane; e < KT * 8; e += 32)
+                                    *reinterpret_cast<uint4 *>(vt + hh * C::BOX + e * 16) = make_uint4(0u, 0u, 0u, 0u);
+                            fence_proxy_async_smem();
+                        }
+                        unsigned bit;
+                        unsigned *word = bars->ring.bad_word(it, pc, j, bit);
+                        clean_rows<C::HALVES, C::BOX, 4>(vt, 0, t.n, word, bit);
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&bars->v_full[st]);
+                    }
                 }
             }
         }
@@ -394,7 +489,7 @@ packed_tc32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                 const int e = me + CONV * i, row = e / CH, c = e % CH;
                 uint32_t w[3][4];
 #pragma unroll
-                for (int k = 0; k < 4; ++k) split3(x[i][2 * k], x[i][2 * k + 1], w[0][k], w[1][k], w[2][k]);
+                for (int k = 0; k < 4; ++k) split3_cache(x[i][2 * k], x[i][2 * k + 1], w[0][k], w[1][k], w[2][k]);
                 if (slot) load(i, next, tn);
                 uint8_t *at = tile + (c >> 3) * C::BOX + row * 128 + (((c & 7) ^ (row & 7)) << 4);
 #pragma unroll
@@ -452,7 +547,7 @@ packed_tc32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
             for (int j = pc.j0;; ++j) {
                 const bool more = j < pc.j1;
                 uint32_t sr[KH];
-                float alpha = 1.f;
+                float alpha = 1.f, sum = 0.f;
                 bool grow = false;
                 if (more) {
                     ok = __all_sync(0xffffffffu, mbar_wait(&bars->s_full, js & 1, p.err, abort_flag));
@@ -499,8 +594,8 @@ packed_tc32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                         sr[c] = __float_as_uint(e.x);
                         sr[c + 1] = __float_as_uint(e.y);
                     }
-                    const float2 sum = fadd2(acc[0], acc[1]);
-                    l += sum.x + sum.y;
+                    const float2 sums = fadd2(acc[0], acc[1]);
+                    sum = sums.x + sums.y;
                     ++js;
                 } else {
                     // every S of this piece has been read (s_full of the last one, and its exchange): the
@@ -527,6 +622,23 @@ packed_tc32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                     }
                 }
                 if (!more) break;
+                // A weight that is not a number over a bf16 cache: the parts of q times an infinite key cancel.
+                if (!KV32 && __builtin_expect(__any_sync(0xffffffffu, sum != sum && l == l), 0)) {
+                    const TileAt t = tile_at(pc, j);
+                    uint32_t w[KH];  // in local memory, to keep this path short
+#pragma unroll
+                    for (int c = 0; c < KH; ++c) w[c] = sr[c];
+                    float kept = sum;
+                    const bool lost = sum != sum && l == l && (r >> p.lg_g) < pc.ntok;
+                    const int64_t row = (int64_t)(pc.tok0 + (lost ? r >> p.lg_g : 0)) * p.nHead + (pc.g << p.lg_g) + (r & ((1 << p.lg_g) - 1));
+                    if (keep_weights<D, KH, KV>(w, lost, reinterpret_cast<const float *>(p.q) + row * D,
+                                                reinterpret_cast<const KV *>(t.pre ? p.pk : p.k) + (t.row + half * KH) * D, kept)) {
+                        sum = kept;
+#pragma unroll
+                        for (int c = 0; c < KH; ++c) sr[c] = w[c];
+                    }
+                }
+                l += sum;
 #pragma unroll
                 for (int c = 0; c < KH / 32; ++c) {
                     uint32_t a[16], b[16], d[16];
@@ -547,7 +659,7 @@ packed_tc32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
             ok = exchange(l, lo);
             if (!ok) break;
             l = half == 0 ? l + lo : lo + l;  // the same sum in both halves
-            redo_row<D, DH, true, float, KV>(p, pc, r, half * DH, scale, m, l, o);
+            put_back<D, DH, !KV32, KV>(p, pc, bars->ring.bad[it % kRing], bars->ring.bad_step(pc), r, half * DH, o);
             ok = finish_rows<D, DH, float, BM>(p, cut, pc, half, r, half * DH, o, m, l, group_sync, &bars->last_flag[half],
                                                base + C::OFF_STG + (warp - C::SOFT0) * 32 * kStgRow);
             bars->ring.put(it, lane);

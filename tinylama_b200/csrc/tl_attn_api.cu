@@ -1354,7 +1354,7 @@ int tl_prefill_packed(tl_attn *h, int layer, int slot0, int nseq, int ntok, cons
     if (ntok < 0) return fail(TL_ERR_INVALID, "negative number of rows");
     if (!aligned(q, 16) || !aligned(out, 16)) return fail(TL_ERR_INVALID, "q and out must be 16-byte aligned");
     if (ntok == 0) return TL_OK;
-    // a row that is summed again (redo_row) reads its q while other threads store their part of its output
+    // rows of one unit are stored while q of others is still to be read
     const size_t bytes = (size_t)ntok * h->nHead * h->headDim * (ioType == TL_IO_BF16 ? 2 : 4);
     const uintptr_t q0 = reinterpret_cast<uintptr_t>(q), o0 = reinterpret_cast<uintptr_t>(out);
     if (q0 < o0 + bytes && o0 < q0 + bytes) return fail(TL_ERR_INVALID, "q and out overlap");
