@@ -186,6 +186,12 @@ template <> struct KvT<__nv_bfloat16> {
     __device__ __forceinline__ static __nv_bfloat16 from_f(float x) { return __float2bfloat16_rn(x); }
 };
 
+// two values rounded to bf16, the first in the low half
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+
 // Load VPL consecutive KV elements from shared memory as floats.
 template <typename T, int VPL> struct VecLoad;
 template <> struct VecLoad<float, 4> {

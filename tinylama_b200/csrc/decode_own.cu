@@ -66,7 +66,7 @@ struct Cursor {
 __device__ __forceinline__ uint32_t third2(float x0, float x1, uint32_t hi, uint32_t lo) {
     auto low = [](uint32_t u) { return __uint_as_float(u << 16); };
     auto high = [](uint32_t u) { return __uint_as_float(u & 0xffff0000u); };
-    return pack2(x0 - low(hi) - low(lo), x1 - high(hi) - high(lo));
+    return pack_bf16(x0 - low(hi) - low(lo), x1 - high(hi) - high(lo));
 }
 
 // The state of one head over a job's n positions (rows k, v) by fp32 products, for one whose sums have

@@ -41,15 +41,11 @@ __device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&v);
-}
 // bf16 hi/lo split of a pair: x = hi + lo with |lo| <= 2^-9 |x|, both bf16
 __device__ __forceinline__ void split2(float x0, float x1, uint32_t &hi, uint32_t &lo) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(x0, x1);
     hi = *reinterpret_cast<const uint32_t *>(&h);
-    lo = pack2(x0 - __low2float(h), x1 - __high2float(h));
+    lo = pack_bf16(x0 - __low2float(h), x1 - __high2float(h));
 }
 
 // D += A * B, m16n8k8, tf32 inputs, fp32 accumulators (f32 caches).  A rows 0..7 carry the

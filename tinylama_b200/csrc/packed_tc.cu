@@ -78,14 +78,6 @@ struct PkBars {
     volatile unsigned lead[4];  // by scheduler: how far group 0's exponentials are, kLeadUnit a piece
 };
 
-__device__ __forceinline__ void tma_load(void *dst, const CUtensorMap *map, int x, int y, uint64_t *bar, uint32_t issue) {
-    asm volatile(
-        "{\n\t.reg .pred e;\n\t"
-        "setp.ne.b32 e, %5, 0;\n\t"
-        "@e cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n\t}" ::
-            "r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar)), "r"(issue)
-        : "memory");
-}
 __device__ __forceinline__ void tma_load3(void *dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar,
                                           uint32_t issue) {
     asm volatile(
@@ -225,7 +217,7 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                     __syncwarp();
 #pragma unroll
                     for (int hh = 0; hh < S_::HALVES; ++hh)
-                        tma_load(sK + st * S_::TILE + hh * S_::BOX, km, 64 * hh, row, &bars->k_full[st], leader);
+                        tma_load_2d(sK + st * S_::TILE + hh * S_::BOX, km, 64 * hh, row, &bars->k_full[st], leader);
                     if (!wait_all(&bars->v_empty[st], par, p.err, abort_flag)) {
                         // K of this stage is in flight, V is not: wait for the K alone
                         wait_all(&bars->k_full[st], (kvit / NS) & 1, nullptr, nullptr);
@@ -236,7 +228,7 @@ packed_tc_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
                     __syncwarp();
 #pragma unroll
                     for (int hh = 0; hh < S_::HALVES; ++hh)
-                        tma_load(sV + st * S_::TILE + hh * S_::BOX, vm, 64 * hh, row, &bars->v_full[st], leader);
+                        tma_load_2d(sV + st * S_::TILE + hh * S_::BOX, vm, 64 * hh, row, &bars->v_full[st], leader);
                 }
             }
             pc.w = -1;
@@ -545,10 +537,6 @@ cudaError_t launch_t(const PackedArgs &a, cudaStream_t s) {
     kern<<<a.ctas, kThreads, smem, s>>>(qm, km, vm, pkm, pvm, p);
     return cudaGetLastError();
 }
-
-}  // namespace
-
-namespace {
 
 // One warp per row, a lane holding D/32 columns.  Few rows, so each row's parts are loaded
 // together (up to 8 in flight) before they are added.

@@ -88,15 +88,6 @@ struct P32Bars {
     float xch[2][2][BM];  // a row's maximum (or sum) over each half of the keys, two turns of it
 };
 
-__device__ __forceinline__ void tma_load(void *dst, const CUtensorMap *map, int x, int y, uint64_t *bar, uint32_t issue) {
-    asm volatile(
-        "{\n\t.reg .pred e;\n\t"
-        "setp.ne.b32 e, %5, 0;\n\t"
-        "@e cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];\n\t}" ::
-            "r"(smem_u32(dst)), "l"(map), "r"(x), "r"(y), "r"(smem_u32(bar)), "r"(issue)
-        : "memory");
-}
-
 // one K = 16 step, A from TMEM
 __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate,
                                        uint32_t issue) {
@@ -288,7 +279,7 @@ packed_tc32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                         __syncwarp();
 #pragma unroll
                         for (int hh = 0; hh < C::HALVES; ++hh)
-                            tma_load(sK + st * C::TILE + hh * C::BOX, km, 64 * hh, (int)t.row, &bars->k_full[st], leader);
+                            tma_load_2d(sK + st * C::TILE + hh * C::BOX, km, 64 * hh, (int)t.row, &bars->k_full[st], leader);
                         if (!wait_all(&bars->v_empty[st], par, p.err, abort_flag)) {
                             wait_all(&bars->k_full[st], (kvit / NS) & 1, nullptr, nullptr);  // the K in flight
                             ok = false;
@@ -298,7 +289,7 @@ packed_tc32_kernel(const __grid_constant__ CUtensorMap kmap, const __grid_consta
                         __syncwarp();
 #pragma unroll
                         for (int hh = 0; hh < C::HALVES; ++hh)
-                            tma_load(sV + st * C::TILE + hh * C::BOX, vm, 64 * hh, (int)t.row, &bars->v_raw[st], leader);
+                            tma_load_2d(sV + st * C::TILE + hh * C::BOX, vm, 64 * hh, (int)t.row, &bars->v_raw[st], leader);
                     }
                 }
             }

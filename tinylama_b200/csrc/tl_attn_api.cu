@@ -234,7 +234,7 @@ Plan plan_decode(const tl_attn *h, int nseq, const int *pos_host, int pos_offset
                  bool cluster_ok = false, bool exchange = false) {
     const int G = h->nHead / h->nHeadKv;
     const int occ = decode_ctas_per_sm(h->headDim, G, h->kvDtype, nseq);
-    const int ctas = h->numSms * occ;  // sms: where the launch shares the device
+    const int ctas = h->numSms * occ;
     long long tot = 0;
     int nmax = 0;
     std::vector<int> ns(nseq);
@@ -622,12 +622,14 @@ SharedPlan plan_shared(const tl_attn *h, int nseq, const int *pos_host, int pref
     return best;
 }
 
-// Chunks of the own positions: two jobs for each of the own kernel's warps (three for an f32 cache, whose
-// tiles take longer: 47 us against 49 at 48 sequences of up to 300, and 37 against 35 the other way
-// round at 64 of up to 512 in bf16), at least 64 positions (a
-// state of headDim + 2 floats then stays well below the keys it stands for) and at most 192 (more jobs
-// even out the warps: 141 us against 146 with whole sequences, 256 of up to 1024), but no more than 16 chunks,
-// so that the states of a long cache stay few.
+// Chunks of the own positions.
+//  * Two jobs for each of the own kernel's warps, three for an f32 cache, whose tiles take longer: 48
+//    sequences of up to 300 (f32, 32/8/128) take 47 us with three and 49 with two; 64 of up to 512 (bf16) 35 with two
+//    and 37 with three.
+//  * At least 64 positions: the state that a chunk leaves, headDim + 2 floats a head, then stays well below the keys
+//    that it stands for.
+//  * At most 192: more jobs even out the warps (256 sequences of up to 1024: 141 us, 146 with whole sequences).
+//  * No more than 16 to a sequence, so that a long cache leaves few states.
 constexpr int kMaxChunks = 16, kOwnWarps = 6;
 constexpr int kMaxSharedSeqs = 4000;  // two ints for each stay in the own kernel's shared memory
 void own_chunks(const tl_attn *h, int nseq, const int *pos_host, int sms, int *chunk, int *nchunks) {
