@@ -163,7 +163,9 @@ TL_API int tl_decode_step(tl_attn *h, int layer, int slot0, int nseq, const int 
                    const int *pos_host, float *q, float *k, const float *v, float *out,
                    void *stream);
 /* Attention only (no RoPE, no append): q already rotated, cache already holds positions
- * 0..pos_dev[b]. */
+ * 0..pos_dev[b].  What the slot holds behind them does not matter, infinities and NaN included (the
+ * same for tl_decode_step and tl_prefill_step); within them, such a value may make the sequence's
+ * whole result NaN. */
 TL_API int tl_decode_attention(tl_attn *h, int layer, int slot0, int nseq, const int *pos_dev,
                         const int *pos_host, const float *q, float *out, void *stream);
 /* Batched prefill from position 0 (src/forward.nim:271-274 per sequence): q

@@ -21,7 +21,7 @@
 //   D = 128:  S (128, taken in turns by the two tiles), P0 P1, O0 O1 (128 each)
 // What bounds it is the softmax.  With D = 64 the exponentials of a unit's tile (256 x 128) take 2048 clocks of the
 // MUFU unit, its products 512 of the tensor core; a tile takes about 2950, and a unit 2 to 3.5 us more.  8 documents
-// of up to 4096 (32/8/64): 460 us, 630 TFLOP/s; 6 prompts of up to 4096 behind 1000 shared positions (32/8/128): 685 us, 970
+// of up to 4096 (32/8/64): 465 us, 625 TFLOP/s; 6 prompts of up to 4096 behind 1000 shared positions (32/8/128): 681 us, 980
 // TFLOP/s.  One exponential in 4 or 8 as a polynomial on the FMA pipe was slower (486, 502 us against 461).
 //
 // With D = 128 a tile's S is free again as soon as its group has it in registers, so one S serves both

@@ -31,9 +31,9 @@
 // While the group works on one tile the tensor core has S of the next one to do, and each piece's q
 // is in place before the one ahead has been written out.
 //
-// Measured: 101 us for 4 prompts of up to 1024 (32/4/64), 442 for 8 of up to 2048 (32/8/64), and over a bf16 cache
-// 260 for 4 of up to 2048 (32/8/128); the tensor pipe is 39% busy in the first (55% on the busiest SM), and waits
-// for the parts that the softmax threads write.
+// Measured: 103 us for 4 prompts of up to 1024 (32/4/64), 450 for 8 of up to 2048 (32/8/64), 455 for 4 of up to 2048
+// (32/8/128), and over a bf16 cache 76 for the first and 260 for the last.  The tensor pipe is 36% busy in the
+// first (46% on the busiest SM) and waits for the parts that the softmax threads write.
 //
 // Masked keys and leftovers: V rows that no row of the unit sees are zero in shared memory.  Values of the
 // sequence itself that are not finite: an f32 cache's infinities go through the products as what they are
